@@ -306,7 +306,8 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_residents(D, RW)) void tree_t
       const int32_t id0 = __builtin_amdgcn_readlane(ids[0], lane_at), id1 = __builtin_amdgcn_readlane(ids[1], lane_at);
       const int32_t id = at < 64 ? id0 : id1;
       const uint32_t u = id >= 0 ? static_cast<uint32_t>(id) : 0u;
-      p.k[j] = cache_head + static_cast<uint64_t>(u >> 4) * blk_bytes + (u & 15u) * grp_bytes;
+      // (64 bits: one group fits 32, fifteen need not.)
+      p.k[j] = cache_head + static_cast<uint64_t>(u >> 4) * blk_bytes + static_cast<uint64_t>(u & 15u) * grp_bytes;
     }
     return p;
   };
