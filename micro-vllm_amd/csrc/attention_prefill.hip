@@ -409,7 +409,8 @@ __device__ __forceinline__ void prefill_body(const AttnArgs& a, int32_t lg_tok, 
     // instructions. Byte address of the K page segment with entry id:
     auto page_base = [&](int32_t id) {
       const uint32_t u = static_cast<uint32_t>(id);
-      return cache_head + static_cast<uint64_t>(u >> 4) * blk_bytes + (u & 15u) * grp_bytes;
+      // (64 bits: one group fits 32, fifteen need not.)
+      return cache_head + static_cast<uint64_t>(u >> 4) * blk_bytes + static_cast<uint64_t>(u & 15u) * grp_bytes;
     };
     // Unmapped page (or beyond the last visible key): its V rows are zeroed.
     auto zero_v = [&](int stage) {

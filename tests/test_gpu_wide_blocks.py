@@ -9,6 +9,7 @@ import torch
 
 from _tree_reference import build, check, random_tree
 from micro_vllm_amd.attention.operators.mi355x_tree import hip_tree_attention
+from test_gpu_attention import build_case, operator, run_and_check
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +43,13 @@ def test_trees_over_groups_far_apart(device, dtype, nodes, d, block, token):
     got = hip_tree_attention(b.query, b.key, b.value, wide, b.metadata)
     assert torch.equal(got, expected)
     assert torch.equal(wide.contiguous().view(torch.int16), b.cache.view(torch.int16))
+
+
+@pytest.mark.parametrize(("block", "token"), WIDE, ids=str)
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("qlens", [[200, 33], [70, 1, 2]], ids=["chunks", "mixed"])
+def test_chunks_over_groups_far_apart(device, qlens, d, block, token):
+    q, k, v, cache, md = build_case(device, torch.bfloat16, [300, 500, 40][: len(qlens)], qlens, 8, 2, d, block, seed=6)
+    wide = spread(cache, token)
+    got = run_and_check(q, k, v, wide, md, torch.bfloat16)
+    assert torch.equal(got, operator()(q, k, v, cache, md))
