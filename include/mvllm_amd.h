@@ -473,7 +473,9 @@ int mvllm_resize_block_tables(const mvllm_block_tables* tables,
  *   status[num_requests]            int32, as above
  * A length below the request's new tokens is refused (status 2). A request
  * with another status than 0, or slot -1, gets a null table row, slots -1 and
- * length 0. A node whose parent is neither an earlier node nor -1,
+ * length 0 in these outputs, while its row of `tables` stays: its length before
+ * the call is the caller's to keep (mvllm_resize_block_tables would release the
+ * row for that 0). A node whose parent is neither an earlier node nor -1,
  * or that descends from one, or that is behind the first MVLLM_MAX_TREE_NODES,
  * stands at position C and sees no node. Tokens outside every request get
  * slot -1 and zeros. The query_start_locations ascend.

@@ -259,9 +259,11 @@ def accept_tree(
     ``max_accepted`` (up to 1,024) are taken. ``kv_caches`` (every layer's cache,
     or one tensor with a leading layer dimension; all alike) are changed in
     place: accepted node k's rows go to position cached + k. A request whose
-    context length is below its nodes accepts nothing and keeps that length
-    (``pack_tree`` gives 0 to one that it did not serve: that row's own length
-    is the caller's to keep)."""
+    context length is below its nodes accepts nothing and keeps that length.
+    ``pack_tree`` gives 0 to one that it did not serve; that request's own
+    length is the caller's to keep, ``torch.where(status == 0,
+    accepted.context_lengths, cached)`` with the status of ``pack_tree`` and the
+    cached tokens before the step, as ``resize`` would release its row for 0."""
 
     device = draft_tokens.device
     if device.type != "cuda":

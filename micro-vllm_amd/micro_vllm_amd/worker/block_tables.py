@@ -112,8 +112,10 @@ class DeviceBlockTables:
         return _int64(slots, "slots", count, device), _int64(lengths, "lengths", count, device), count
 
     def resize(self, slots: torch.Tensor, lengths: torch.Tensor) -> torch.Tensor:
-        """Grow or cut each request's row to the blocks that ``lengths`` need
-        (0 releases it); returns the status."""
+        """Grow or cut each request's row to the blocks that ``lengths`` need;
+        returns the status. Length 0 releases a row, live or not: after a step,
+        pass a request that ``pack`` or ``pack_tree`` did not serve the length it
+        had before, not the 0 that stands in the step's metadata."""
 
         slots, lengths, count = self._requests(slots, lengths)
         device = self.rows.device
@@ -178,7 +180,8 @@ class DeviceBlockTables:
         """``resize``, and the metadata of a step whose new tokens are the last
         ``query_start_locations[r + 1] - query_start_locations[r]`` of each
         request's ``lengths[r]``. A request that is not served gets a null row,
-        slots -1 and length 0."""
+        slots -1 and length 0 in the metadata; its blocks stay its own, and its
+        length before the call is the caller's to keep."""
 
         if num_tokens < 0:
             raise ValueError("num_tokens must not be negative")
