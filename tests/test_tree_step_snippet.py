@@ -66,13 +66,13 @@ def accept_one(*args, **kwargs):
     )
 
 
-def run_step(tables, cached, sizes):
+def run_step(tables, cached, sizes, forward=lambda *args: None):
     """One pass of the guide's code; returns its namespace."""
 
     namespace = dict(
         DeviceBlockTables=SimpleNamespace(create=lambda *a: tables), FullAttentionSpec=FullAttentionSpec, torch=torch,
         num_blocks=None, num_slots=None, width=WIDTH, block_size=BLOCK, device=None,
-        model=SimpleNamespace(forward=lambda *a, **k: None, logits=lambda hidden: None), argmax_rows=lambda logits: None, logits=None,
+        model=SimpleNamespace(forward=forward, logits=lambda hidden: None), argmax_rows=lambda logits: None, logits=None,
         accept_tree=accept_one, kv_caches=["cache"], drafts=None, first_tokens=torch.zeros(len(sizes), dtype=torch.int64),
         slots=torch.arange(len(sizes)), cached=torch.tensor(cached), sizes=torch.tensor(sizes),
         lengths=torch.tensor(cached) + torch.tensor(sizes), parents=None,
@@ -105,3 +105,15 @@ def test_the_blocks_of_refused_nodes_go_back():
     after = run_step(tables, [30, 33], [40, 1])
     assert tables.packed == [SERVED, SERVED]
     assert after["cached"].tolist() == [31, 34] and tables.model.free == free
+
+
+def test_the_model_is_called_as_it_is_declared():
+    from micro_vllm_amd.harness.model import DecoderModel
+
+    calls = []
+    tables = ListTables(20, 1, WIDTH, BLOCK)
+    tables.model.resize([0], [30])
+    run_step(tables, [30], [4], forward=lambda *args: calls.append(bound(DecoderModel.forward, *args)))
+    (called,) = calls
+    assert called["positions"] == "positions" and called["kv_caches"] == ["cache"]
+    assert hasattr(called["metadata"], "context_lengths")
