@@ -14,10 +14,16 @@
 // v_permlane32_swap, and P^T is the B operand of the second product as it
 // stands. K and V pages of 16 keys go HBM -> LDS directly, a tile and a half
 // ahead. Online softmax in the exp2 domain; the accumulators are rescaled only
-// when a maximum has grown much. Scores, maxima, sums and the output stay fp32; the weights are rounded to the input type, each by at most
-// half a step, and the row sum adds the rounded ones, so they are normalised
-// exactly. In fp16 they are lifted by 2^7: a weight keeps its 11 bits down to
-// 2^-21 of the row's largest.
+// when a maximum has grown much. Scores, maxima, sums and the output stay fp32.
+// The weights enter P.V as two values of the input type, the rounded weight and
+// what it lacks: 16 bits in bf16, 22 in fp16 (lifted by 2^7, so that the second
+// value's subnormals, 2^-24, are 2^-31 of the row's largest weight), as many as
+// the paged decode kernel's pair, whatever else is in the batch. Rounded weights
+// alone left 1.4 times the error of fp32 ones; the pair costs nothing in items of
+// 32 or 64 rows (one request of 8 nodes 12.5 us, 16 of 24-32 48.4, both ways) and
+// a second P.V product where the matrix cores are the bound: 64 requests of 64
+// nodes over 1k-8k keys 377 -> 480 us, 24 of 40-90 in a window 37.6 -> 44.5, 4 of
+// 20-27 over 16k-33k 96 -> 97-109.
 //
 // Which keys a row sees is a 32-bit word per 32 keys: cached positions from its
 // start on, then its mask bits shifted to the tile. Tiles wholly among the
@@ -374,9 +380,9 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_residents(D, RW)) void tree_t
     return v;
   };
 
-  // P^T of 32 keys as MFMA B operands.
+  // P^T of 32 keys as MFMA B operands: the rounded weights, and what they lack.
   struct Weights {
-    short8_t part[2];
+    short8_t part[2][2];
   };
   auto read_k = [&](int hb, int stage, short8_t (&kf)[kSteps]) {
 #pragma unroll
@@ -407,31 +413,37 @@ __global__ __launch_bounds__(64 * kTreeWaves, tree_residents(D, RW)) void tree_t
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? s[i] : -INFINITY;
   };
-  // O^T += V^T . P^T of 32 keys; `between(i)` follows product i of 2 kBlocks.
+  // O^T += V^T . P^T of 32 keys; `between(i)` follows pair i of 2 kBlocks products.
   auto accumulate = [&](const short4v (&vf)[2][kSteps], const Weights& p, auto&& between) {
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
       for (int c = 0; c < kBlocks; ++c) {
         const short4v lo4 = vf[q][c], hi4 = vf[q][kBlocks + c];
-        oacc[c] = Mma32<T>::mma(short8_t{lo4[0], lo4[1], lo4[2], lo4[3], hi4[0], hi4[1], hi4[2], hi4[3]}, p.part[q], oacc[c]);
+        const short8_t av = {lo4[0], lo4[1], lo4[2], lo4[3], hi4[0], hi4[1], hi4[2], hi4[3]};
+        oacc[c] = Mma32<T>::mma(av, p.part[0][q], oacc[c]);
+        oacc[c] = Mma32<T>::mma(av, p.part[1][q], oacc[c]);
         between(q * kBlocks + c);
       }
   };
-  // Weights against the offset `off`; returns this lane's sum of the rounded ones.
+  // Weights against the offset `off`; returns this lane's sum.
   auto weigh = [&](const float16v& s, float off, Weights& p) {
     float sum = 0.f;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      uint32_t w[4];
+      uint32_t w[2][4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * q + 2 * x], a.scale_log2, -off));
         const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * q + 2 * x + 1], a.scale_log2, -off));
-        w[x] = Mma32<T>::pack2(p0, p1);
-        sum = Mma32<T>::dot2_ones(w[x], sum);
+        sum += p0 + p1;
+        w[0][x] = Mma32<T>::pack2(p0, p1);
+        const float2v rest = Mma32<T>::less(p0, p1, w[0][x]);
+        w[1][x] = Mma32<T>::pack2(rest[0], rest[1]);
       }
-      p.part[q] = __builtin_bit_cast(short8_t, uint4{w[0], w[1], w[2], w[3]});
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+        p.part[y][q] = __builtin_bit_cast(short8_t, uint4{w[y][0], w[y][1], w[y][2], w[y][3]});
     }
     return sum;
   };
