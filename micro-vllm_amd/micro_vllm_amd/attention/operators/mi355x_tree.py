@@ -28,6 +28,8 @@ def _tree_attention(
     layer_kv_cache: torch.Tensor,
     metadata: TreeAttentionMetadata,
 ) -> torch.Tensor:
+    if (key is None) != (value is None):
+        raise ValueError("mi355x_tree attention takes key and value together, or neither")
     device, dtype = query.device, query.dtype
     if device.type != "cuda":
         raise RuntimeError("mi355x_tree attention requires GPU tensors")
