@@ -29,6 +29,17 @@ def gpu_available() -> bool:
     return torch.cuda.is_available()
 
 
+@pytest.fixture(autouse=True)
+def no_error_left_behind():
+    """After each test, the library's last error is cleared (by a call that
+    succeeds), so that no test sees what an earlier one was refused for."""
+
+    yield
+    native = sys.modules.get("micro_vllm_amd._native")
+    if native is not None and native.LIBRARY_PATH.exists():
+        native.load().mvllm_tree_attention_workspace_bytes(None, 1, None)
+
+
 @pytest.fixture
 def device():
     """cuda:0. After the test, dead objects are collected while no graph
