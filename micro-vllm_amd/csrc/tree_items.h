@@ -48,17 +48,17 @@ __device__ __forceinline__ TreeReq tree_request(const TreeArgs& a, int64_t r) {
   return q;
 }
 
-__device__ __forceinline__ int64_t tree_load(const TreeReq& q) {
+__host__ __device__ __forceinline__ int64_t tree_load(const TreeReq& q) {
   return static_cast<int64_t>(q.blocks) * (q.keys > 0 ? q.keys : 1);
 }
 
-__device__ __forceinline__ int32_t tree_splits(const TreeArgs& a, const TreeReq& q, int32_t split) {
+__host__ __device__ __forceinline__ int32_t tree_splits(const TreeArgs& a, const TreeReq& q, int32_t split) {
   return a.merge_capacity > 0 && q.keys > split ? (q.keys + split - 1) / split : 1;
 }
 
 // Keys of each of a request's `ns` splits but the last: even shares, at most the
 // split length that gave ns, so that the last one has keys as well.
-__device__ __forceinline__ int32_t tree_share(const TreeReq& q, int32_t ns) {
+__host__ __device__ __forceinline__ int32_t tree_share(const TreeReq& q, int32_t ns) {
   return ns > 1 ? ((q.keys + ns - 1) / ns + 63) & ~63 : q.keys;
 }
 
@@ -103,29 +103,38 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+// 1 / x to a unit in the last place.
+__host__ __device__ __forceinline__ float reciprocal(float x) {
+#ifdef __HIP_DEVICE_COMPILE__
+  return __builtin_amdgcn_rcpf(x);
+#else
+  return 1.0f / x;
+#endif
+}
+
 // Split lengths to choose from, for `total` keys over all row blocks: attempt c
 // shares them among (16 - c) / 16 of the workgroups that run at once, the last
 // one among half. Keys are summed in fp32 and divided by reciprocals: each length
 // is longer by more than their rounding (2^-14 relative to a few times 2^-22).
 constexpr int kAttempts = 8;
-__device__ __forceinline__ float split_share(const TreeArgs& a, float total) {
-  return total * __builtin_amdgcn_rcpf(static_cast<float>(a.target)) * (16.0f + 0.001f);
+__host__ __device__ __forceinline__ float split_share(const TreeArgs& a, float total) {
+  return total * reciprocal(static_cast<float>(a.target)) * (16.0f + 0.001f);
 }
-__device__ __forceinline__ int32_t split_length(const TreeArgs& a, float share, int c) {
-  const float x = fmaxf(share * __builtin_amdgcn_rcpf(static_cast<float>(16 - c)) + 1.0f, static_cast<float>(a.shortest));
+__host__ __device__ __forceinline__ int32_t split_length(const TreeArgs& a, float share, int c) {
+  const float x = fmaxf(share * reciprocal(static_cast<float>(16 - c)) + 1.0f, static_cast<float>(a.shortest));
   return x < static_cast<float>(kFar) ? (static_cast<int32_t>(x) + 63) & ~63 : kFar;
 }
 
 // Items of `blocks` row blocks of `keys` keys in splits of `length`, at least
 // (1 / length is rounded up: a quotient just below an integer counts as that).
-__device__ __forceinline__ int32_t split_count(int32_t blocks, int32_t keys, int32_t length) {
-  const float q = static_cast<float>(keys - 1) * (__builtin_amdgcn_rcpf(static_cast<float>(length)) * (1.0f + 0x1p-20f));
+__host__ __device__ __forceinline__ int32_t split_count(int32_t blocks, int32_t keys, int32_t length) {
+  const float q = static_cast<float>(keys - 1) * (reciprocal(static_cast<float>(length)) * (1.0f + 0x1p-20f));
   const int32_t n = static_cast<int32_t>(q) + 1;
   return blocks * (n > 1 ? n : 1);
 }
 
 // Whether the shortest split leaves no more items than run at once.
-__device__ __forceinline__ bool all_shortest(const TreeArgs& a, float total, float blocks) {
+__host__ __device__ __forceinline__ bool all_shortest(const TreeArgs& a, float total, float blocks) {
   const float shortest = static_cast<float>(a.shortest);
   return total + blocks * shortest <= static_cast<float>(a.target) * shortest;
 }
