@@ -215,8 +215,9 @@ int mvllm_attention_forward(const mvllm_tensor3* query,
  * 64 * mask_words is refused. max_query_len (<= 0: unknown) only chooses the
  * kernel's shape. With key and value (both or neither), the nodes' rows are
  * first written to slot_mapping, as by mvllm_kv_write, where no other request of
- * the call may read them; without, the cache holds them already. Positions stay below 2^30, head_dim up to 512, scale positive.
- * The workspace
+ * the call may read them (the writes are ordered before their own request's
+ * reads only); without, the cache holds them already. Positions stay below
+ * 2^30, head_dim up to 512, scale positive. The workspace
  * (mvllm_tree_attention_workspace_bytes; 16-byte aligned) needs no
  * initialisation and holds nothing between calls; calls that overlap need one
  * each. Graph-capturable.

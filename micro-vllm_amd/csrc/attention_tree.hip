@@ -28,7 +28,10 @@ __device__ __forceinline__ int64_t owner_of(const TreeArgs& a, int64_t t) {
 // One workgroup of four waves per (node, query head): each wave takes every
 // fourth block of 64 keys, a lane scores one key, then the lanes hold the
 // output's dims. Only visible keys are read, so nothing that a masked row
-// holds can reach the output.
+// holds can reach the output. Bound by its loads: a lane reads its key's row one
+// element at a time, and neither nodes nor heads share what they read. 4 requests
+// of 24 nodes over 2,000 keys, 32/8 heads, bf16: 1,139 us at head_dim 80, 1,630 at
+// 128 in blocks of 8 (the tile kernel takes 26 in blocks of 16).
 constexpr int kAnyWaves = 4;
 
 template <typename T, int DPL>

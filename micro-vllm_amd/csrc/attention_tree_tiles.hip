@@ -794,7 +794,8 @@ int64_t tree_tiles_layout(TreeArgs& a, int64_t max_nodes, void* workspace) {
   const int rw = most <= 32 ? 1 : (most <= 64 ? 2 : 4);
   // Splits of 384 keys or more: 32 nodes of one request over 2,000 keys take 20.5
   // us so, 25.6 with 512 and 20.3 with 128, but a table that holds no more than
-  // 384 keys needs no merge (12.3 us for 8 nodes over 320 instead of 13.4).
+  // 384 keys needs no merge (12.3 us for 8 nodes over 320 instead of 13.4; a wider
+  // table has its merge launched whatever the lengths, which the host does not know).
   return tree_layout(a, 32 * rw, 384, tree_residents(a.head_dim, rw), workspace);
 }
 

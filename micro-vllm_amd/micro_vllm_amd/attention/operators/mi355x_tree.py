@@ -4,7 +4,10 @@ Attention of drafted trees over the paged cache, with the call and error
 conventions of ``"mi355x_paged"``: the same positional signature, the nodes'
 K/V written in place, a new output tensor like ``query``; tensors off the GPU
 raise ``RuntimeError``, unsupported types ``ValueError``. It takes a
-``TreeAttentionMetadata``. All work runs in the HIP library on the current
+``TreeAttentionMetadata``. Unlike there, the rows that a call writes may be read
+by no other request of the same call: a workgroup writes those that it reads, and
+is not ordered with the others. (``DeviceBlockTables`` gives every request blocks
+of its own.) All work runs in the HIP library on the current
 torch stream without host synchronisation, so a call can be captured in a HIP
 graph.
 """
@@ -101,7 +104,11 @@ def hip_tree_attention(
     layer_kv_cache: torch.Tensor,
     metadata: TreeAttentionMetadata,
 ) -> torch.Tensor:
-    """Write the nodes' K/V, then attention over cached tokens and trees."""
+    """Write the nodes' K/V, then attention over cached tokens and trees.
+
+    A slot that this call writes is read by its own request only; where another
+    one's table names it, write the rows first (``hip_write_kv_cache``) and use
+    ``hip_tree_attention_over_cache``."""
 
     return _tree_attention(query, key, value, layer_kv_cache, metadata)
 

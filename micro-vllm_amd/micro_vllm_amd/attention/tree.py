@@ -24,7 +24,8 @@ class TreeAttentionMetadata:
     depth), for the rotary embedding. It sees the cached positions from
     ``query_context_start_positions`` on, and the nodes whose bits are set in
     its row of ``tree_mask`` (int64, 64 nodes per word; its own bit is not
-    implied).
+    implied). ``slot_mapping`` names slots that no other request of the call
+    reads, where the call writes them.
     """
 
     query_positions: torch.Tensor
